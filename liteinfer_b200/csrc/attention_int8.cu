@@ -57,6 +57,7 @@ struct Int8AttnParams {
   float softcap;            // 0: none
   const float* sink;        // [heads] or null: exp(sink[h]) is one more term of head h's denominator
   bool beside;              // the kernel ahead neither writes what this one reads nor the same results: they run side by side
+  bool after_append;        // the kernel ahead is rope_kv_write_int8, and it brings no more than the newest token of these sequences
 };
 
 __device__ __forceinline__ uint4 shared16(unsigned addr) {
@@ -134,8 +135,11 @@ __device__ __forceinline__ void attend(const Int8AttnParams& p, int splits) {
   constexpr unsigned kGroupBytes = 16 * D * 2;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Int8Merge<D, kRows>& merge = *reinterpret_cast<Int8Merge<D, kRows>*>(smem_raw);      // where the rings were
-  // Up to the wait below, a block reads what the kernel ahead of it cannot write: the batch, and pages that do not hold the newest
-  // token (rope_kv_write_int8 lets this kernel start only when all that came before it is done).  q and the newest page come later.
+  // Behind an append of one token a sequence a block starts with what that append cannot write: the batch, and pages that do not hold the
+  // newest token (rope_kv_write_int8 lets this kernel start only when all that came before it is done).  q and the newest page come later.
+  // Behind anything else nothing is read before the kernels ahead are done: an append of several tokens writes the pages before
+  // the newest too, and a kernel that lets its followers start before its own wait passes on what is not done yet.
+  if (!p.beside && !p.after_append) grid_dependency_wait();
   const int seq = p.seq_index ? p.seq_index[blockIdx.z] : blockIdx.z;
   if (seq < 0) return;                          // a place of padding (the whole cluster's)
   const int q_begin = p.query_start_loc[seq];
@@ -685,6 +689,7 @@ struct AttentionInt8Args {
   const float* sink;
   long long splits;         // 1, 2, 4 or 8 blocks share a sequence's keys
   long long beside;         // the kernel ahead on the stream is the same step's li_attention_int8_prompt
+  long long after_append;   // the kernel ahead on the stream is li_rope_kv_write_int8 and writes one token at most of each of these sequences
   cudaStream_t stream;
 };
 
@@ -703,7 +708,7 @@ LI_EXPORT int li_attention_int8(const AttentionInt8Args* a) {
   Int8AttnParams p{a->q, (int)a->q_row_stride, a->out, (int)a->out_row_stride, (const signed char*)a->k_pool, (const signed char*)a->v_pool,
                    a->k_scale, a->v_scale, a->block_table, (int)a->table_stride, a->query_start_loc, a->context_lens, a->seq_index,
                    (int)a->heads, (int)a->kv_heads, (int)a->page_size, (int)a->num_pages, (float)a->scale, (int)a->window,
-                   (float)a->softcap, a->sink, a->beside != 0};
+                   (float)a->softcap, a->sink, a->beside != 0, a->after_append != 0};
   if (a->dtype == kFloat32)
     return a->head_dim == 64 ? launch_heads<float, 64>(p, num_seqs, splits, a->stream) : launch_heads<float, 128>(p, num_seqs, splits, a->stream);
   return a->head_dim == 64 ? launch_heads<bf16, 64>(p, num_seqs, splits, a->stream) : launch_heads<bf16, 128>(p, num_seqs, splits, a->stream);

@@ -31,7 +31,7 @@ _k._SIGNATURES.update({
 })
 _ROPE_KV_WRITE = struct.Struct("=21qdq").pack
 _READ_PAGES = struct.Struct("=22q").pack
-_ATTENTION = struct.Struct("=20qdqd4q").pack
+_ATTENTION = struct.Struct("=20qdqd5q").pack
 _ATTENTION_PROMPT = struct.Struct("=22qd2qd5q").pack
 _QUANTISE_ROWS = struct.Struct("=9q").pack
 _LINEAR = struct.Struct("=17q").pack
@@ -147,8 +147,12 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
                          query_start_loc: torch.Tensor, context_lens: torch.Tensor, num_seqs: int, max_q_len: int, heads: int,
                          kv_heads: int, head_dim: int, scale: float, window: int = 0, plan=None,
                          decode_splits: int | None = None, keep_first: int = 0, softcap: float = 0.0,
-                         sink: torch.Tensor | None = None, chunk: int = 0) -> torch.Tensor:
+                         sink: torch.Tensor | None = None, chunk: int = 0, after_append: bool = False) -> torch.Tensor:
     """`paged_attention` over pages of 8 bits; arguments as there (keys and values of one size).
+
+    `after_append`: the caller says that the launch ahead of this one on the stream is a `rope_kv_write_int8`, and that it wrote one token
+    at most of every sequence that is attended as a single token (a step of the engine).  Their older pages are then read while that
+    launch still writes the newest ones.  After an append of several of a sequence's tokens it would be wrong.
 
     Single tokens (with a `plan`, or where no sequence brings more than one) of head size 64 or 128, groups of at most 16 heads and
     pages of a multiple of 16 tokens read the pages as they are; `decode_splits` blocks share a sequence's keys (rounded down to a
@@ -194,7 +198,7 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
             sequences, prompts, most_queries, heads, kv_heads, head_dim, page_size, num_pages, scale, span, kept, softcap,
             0 if sink is None else sink.data_ptr(), work.data_ptr(), blocks, _k.scratch_for(q.device).gemm_error.data_ptr(), stream)),
             "paged_attention_int8")
-        prompts, beside = 0, True       # (the single tokens' kernel need not wait for this one)
+        prompts, beside = 0, most_queries > 0 and blocks > 0       # (the single tokens' kernel need not wait for this one, if there is one)
     # (Where `paged_attention` takes all sequences in one launch, it takes the single tokens next to portions too.)
     every = plan is None or not _k.mma_attention_supports(dtype, heads, kv_heads, head_dim)
     if singles and direct and (plan is None or not prompts or not every):
@@ -207,7 +211,7 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
         _check(_fn("li_attention_int8")(_ATTENTION(
             code, q.data_ptr(), q_row_stride, out.data_ptr(), out.stride(0), k, v, k_scale, v_scale, table, stride, starts, contexts,
             sequences, singles, heads, kv_heads, head_dim, page_size, num_pages, scale, span, softcap,
-            0 if sink is None else sink.data_ptr(), splits, beside, stream)), "paged_attention_int8")
+            0 if sink is None else sink.data_ptr(), splits, beside, after_append, stream)), "paged_attention_int8")
         singles = 0
     if not prompts and not singles:
         return out

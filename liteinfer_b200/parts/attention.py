@@ -286,7 +286,7 @@ class Attention:
                                    cos_sin_scale=rotary.attention_scaling)
             ops.paged_attention_int8(qkv, qkv.stride(0), attended, kv.int8, table, ctx.query_start_loc, ctx.context_lens, ctx.num_seqs,
                                      ctx.max_query_len, self.heads, self.kv_heads, self.head_dim, self.scale, self.window or 0,
-                                     plan=ctx.plan, decode_splits=ctx.decode_splits, chunk=self.chunk or 0, **masked)
+                                     plan=ctx.plan, decode_splits=ctx.decode_splits, chunk=self.chunk or 0, after_append=True, **masked)
             return
         prepared = self.qk_norm == "head" or self.head_gate or self.output_gate or self.value_mix
         if self.qk_norm and not prepared and not self.joint_norm:
