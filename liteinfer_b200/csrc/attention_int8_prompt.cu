@@ -717,9 +717,11 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
 #pragma unroll
         for (int i = 0; i < kMostSplits; ++i) {
-          const bool some = w[i] != -INFINITY;
-          w[i] = some ? exp2f(w[i] - top) : 0.f;
-          if (some) l += w[i] * remote((D + 1) * kRows + row, i);
+          // A block that saw no key brings neither a reference nor a sum.  One whose scores are all NaN brings no reference either (a maximum
+          // passes NaN over), but its sum is NaN, and so is the row.
+          const float sum = i < splits ? remote((D + 1) * kRows + row, i) : 0.f;
+          w[i] = w[i] != -INFINITY ? exp2f(w[i] - top) : sum == 0.f ? 0.f : NAN;
+          if (w[i] != 0.f) l += w[i] * sum;
         }
         const int qi = q0 + row / groups, head = kvh * groups + row % groups;
         if (p.sink != nullptr) l += exp2f(p.sink[head] * kLog2eF - top);
