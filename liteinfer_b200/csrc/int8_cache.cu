@@ -312,17 +312,28 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
   }
 }
 
-// The same for a rotary width that is no multiple of 16: a block a token, a number at a time.
-template <typename T>
-__device__ __forceinline__ float rotated(const T* row, int j, int half, const float* cosv, const float* sinv) {
-  if (j < half) return rotate_lo(to_float(row[j]), to_float(row[j + half]), cosv[j], sinv[j]);
-  if (j < 2 * half) return rotate_hi(to_float(row[j - half]), to_float(row[j]), cosv[j - half], sinv[j - half]);
-  return to_float(row[j]);
+// The same for a rotary width that is no multiple of 16, and for pages whose tokens' cosines and sines fit no shared memory: a block a token, a
+// number at a time.  kAngles: they do fit; else each is computed where it is used.
+template <bool kAngles, typename T>
+__device__ __forceinline__ float rotated(const AppendParams& p, const T* row, int j, int half, int pos, const float* cosv) {
+  if (j >= 2 * half) return to_float(row[j]);
+  const int i = j < half ? j : j - half;
+  float c, s;
+  if constexpr (kAngles) {
+    c = cosv[i];
+    s = cosv[half + i];
+  } else {
+    const float angle = __fmul_rn((float)pos, p.inv_freq[i]);
+    c = cosf(angle) * p.cs_scale;
+    s = sinf(angle) * p.cs_scale;
+  }
+  const float a = to_float(row[i]), b = to_float(row[i + half]);
+  return j < half ? rotate_lo(a, b, c, s) : rotate_hi(a, b, c, s);
 }
 
-template <typename T>
+template <typename T, bool kAngles>
 __global__ void __launch_bounds__(kAppendWarps * 32) rope_kv_write_int8_odd_kernel(const AppendParams p) {
-  extern __shared__ float shared[];      // cosines and sines of the item's positions: [page_size][2][half]
+  extern __shared__ float shared[];      // kAngles: cosines and sines of the item's positions: [page_size][2][half]
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = p.inv_freq != nullptr ? p.rotary_dim / 2 : 0, D = p.head_dim;
   grid_dependency_wait();
@@ -333,13 +344,15 @@ __global__ void __launch_bounds__(kAppendWarps * 32) rope_kv_write_int8_odd_kern
   if (page >= 0)
     while (t + count < p.tokens && !starts_item(p, t + count, p.positions[t + count], p.seq_of_token[t + count])) ++count;
   const int turns = max(count, 1);
-  for (int i = threadIdx.x; i < turns * half; i += blockDim.x) {
-    const int n = i / half, j = i - n * half;
-    const float angle = __fmul_rn((float)(pos + n), p.inv_freq[j]);
-    shared[n * 2 * half + j] = cosf(angle) * p.cs_scale;
-    shared[n * 2 * half + half + j] = sinf(angle) * p.cs_scale;
+  if (kAngles) {
+    for (int i = threadIdx.x; i < turns * half; i += blockDim.x) {
+      const int n = i / half, j = i - n * half;
+      const float angle = __fmul_rn((float)(pos + n), p.inv_freq[j]);
+      shared[n * 2 * half + j] = cosf(angle) * p.cs_scale;
+      shared[n * 2 * half + half + j] = sinf(angle) * p.cs_scale;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const T* row0 = (const T*)p.qkv + (size_t)t * p.row_stride;
   T* q_out = (T*)p.q_out + (size_t)t * p.q_out_stride;
   // (q may be rotated in place: a warp reads a head whole before it writes it, at most 512 dimensions of it)
@@ -347,7 +360,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) rope_kv_write_int8_odd_kern
     const T* src = row0 + (size_t)h * D;
     T* dst = q_out + (size_t)h * D;
     float r[16];
-    for (int i = 0, j = lane; j < D; j += 32, ++i) r[i] = rotated(src, j, half, shared, shared + half);
+    for (int i = 0, j = lane; j < D; j += 32, ++i) r[i] = rotated<kAngles>(p, src, j, half, pos, shared);
     __syncwarp();
     for (int i = 0, j = lane; j < D; j += 32, ++i) dst[j] = from_float<T>(r[i]);
   }
@@ -359,7 +372,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) rope_kv_write_int8_odd_kern
     unsigned top = 0;
     for (int n = 0; n < count; ++n)
       for (int j = lane; j < D; j += 32)
-        top = max(top, abs_bits(rotated(src + n * p.row_stride, j, turned, shared + n * 2 * half, shared + n * 2 * half + half)));
+        top = max(top, abs_bits(rotated<kAngles>(p, src + n * p.row_stride, j, turned, pos + n, shared + n * 2 * half)));
     const float need = scale_of(warp_max_bits(top));
     float* at = p.scale[which] + (size_t)page * p.kv_heads + h;
     const float old = slot > 0 ? *at : 0.f, scale = grown_scale(old, need);
@@ -371,8 +384,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) rope_kv_write_int8_odd_kern
     const bool holds = scale_holds(scale);
     for (int n = 0; n < count; ++n)
       for (int j = lane; j < D; j += 32)
-        out[(slot + n) * D + j] = (signed char)quantised(
-            rotated(src + n * p.row_stride, j, turned, shared + n * 2 * half, shared + n * 2 * half + half), scale, holds);
+        out[(slot + n) * D + j] = (signed char)quantised(rotated<kAngles>(p, src + n * p.row_stride, j, turned, pos + n, shared + n * 2 * half), scale, holds);
     __syncwarp();
     if (lane == 0) *at = scale;
   }
@@ -457,38 +469,56 @@ struct RopeKvWriteInt8Args {
   cudaStream_t stream;
 };
 
-// head_dim a multiple of 16, at most 512.
+// The most bytes of cosines and sines in a block of rope_kv_write_int8_kernel: what leaves an SM its blocks, and, for pages that need more, what a block
+// may have.
+constexpr size_t kAngleBytes = 40 * 1024, kMostAngleBytes = 200 * 1024;
+
+template <typename T, int kWarps>
+static int launch_append(const AppendParams& p, int chunk, dim3 grid, size_t shared, cudaStream_t stream) {
+  static bool configured = false;
+  if (shared > kAngleBytes && !configured) {
+    const cudaError_t e = cudaFuncSetAttribute(rope_kv_write_int8_kernel<T, kWarps>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostAngleBytes);
+    if (e != cudaSuccess) return (int)e;
+    configured = true;
+  }
+  return (int)launch_pdl(p.tokens, rope_kv_write_int8_kernel<T, kWarps>, grid, dim3(kWarps * 32), shared, stream, p, chunk);
+}
+template <typename T>
+static int launch_append_odd(const AppendParams& p, cudaStream_t stream) {
+  const size_t shared = (size_t)p.page_size * (p.inv_freq != nullptr ? p.rotary_dim : 0) * sizeof(float);
+  const dim3 grid(p.tokens), block(kAppendWarps * 32);
+  return shared <= 48 * 1024 ? (int)launch_pdl(p.tokens, rope_kv_write_int8_odd_kernel<T, true>, grid, block, shared, stream, p)
+                             : (int)launch_pdl(p.tokens, rope_kv_write_int8_odd_kernel<T, false>, grid, block, 0, stream, p);
+}
+
+// head_dim a multiple of 16, at most 512; pages of any number of tokens.
 LI_EXPORT int li_rope_kv_write_int8(const RopeKvWriteInt8Args* a) {
   const int tokens = (int)a->tokens, head_dim = (int)a->head_dim;
   if (tokens == 0) return 0;
-  if (a->heads < 0 || a->kv_heads < 1 || head_dim < 16 || head_dim % 16 || head_dim > 512 || a->page_size < 1) return LI_ERR_UNSUPPORTED;
+  if (a->heads < 0 || a->kv_heads < 1 || head_dim < 16 || head_dim % 16 || head_dim > 512 || a->page_size < 1 ||
+      a->page_size * head_dim > 0x7fffffffL)
+    return LI_ERR_UNSUPPORTED;
   if (a->inv_freq != nullptr && (a->rotary_dim < 0 || a->rotary_dim % 2 || a->rotary_dim > head_dim)) return LI_ERR_UNSUPPORTED;
   const size_t size = a->dtype == kFloat32 ? 4 : 2;
   if (!aligned16(a->qkv) || !aligned16(a->q_out) || a->row_stride * size % 16 || a->q_out_stride * size % 16 || !aligned16(a->k_pool) ||
       !aligned16(a->v_pool))
     return LI_ERR_ALIGNMENT;
-  const size_t smem = (size_t)a->page_size * (a->inv_freq != nullptr ? a->rotary_dim : 0) * sizeof(float);
-  if (smem > 48 * 1024) return LI_ERR_UNSUPPORTED;
   AppendParams p{a->qkv, (size_t)a->row_stride, a->q_out, (size_t)a->q_out_stride, a->positions, a->seq_of_token, a->block_table,
                  (int)a->table_stride, {(signed char*)a->k_pool, (signed char*)a->v_pool}, {a->k_scale, a->v_scale}, a->inv_freq, tokens,
                  (int)a->heads, (int)a->kv_heads, head_dim, (int)a->rotary_dim, (int)a->page_size, (int)a->num_pages, (float)a->cs_scale};
-  const dim3 block(kAppendWarps * 32);
-  if (a->inv_freq != nullptr && a->rotary_dim % 16)
-    return a->dtype == kFloat32 ? (int)launch_pdl(tokens, rope_kv_write_int8_odd_kernel<float>, dim3(tokens), block, smem, a->stream, p)
-                                : (int)launch_pdl(tokens, rope_kv_write_int8_odd_kernel<bf16>, dim3(tokens), block, smem, a->stream, p);
   // Few tokens are a block each (single tokens are items of their own then, and every SM gets some); the more there are, the more share
-  // a block's start, its cosines and its sines.
+  // a block's start, its cosines and its sines, as far as these fit: a block keeps them for its own tokens and for those that end its last page.
+  const size_t each = (size_t)(a->inv_freq != nullptr ? a->rotary_dim : 0) * sizeof(float), page = a->page_size;
+  const size_t most = page * each <= kAngleBytes ? kAngleBytes : kMostAngleBytes;
+  if (page > kMaxPage || page * each > most || each % 64) return a->dtype == kFloat32 ? launch_append_odd<float>(p, a->stream) : launch_append_odd<bf16>(p, a->stream);
   int chunk = 1;
   while (chunk < kMaxChunk && 3L * tokens > 8L * 148 * chunk) chunk *= 2;
-  const size_t shared = (size_t)(a->page_size + chunk - 1) * (a->inv_freq != nullptr ? a->rotary_dim : 0) * sizeof(float);
-  if (shared > 40 * 1024 || a->page_size > kMaxPage) return LI_ERR_UNSUPPORTED;
+  while (chunk > 1 && (page + chunk - 1) * each > most) chunk /= 2;
+  const size_t shared = (page + chunk - 1) * each;
   const dim3 grid((tokens + chunk - 1) / chunk, a->num_pages > 0 ? 3 : 1);
   const bool few = tokens > 2048 && a->kv_heads <= 4 && a->heads * (head_dim / 16) <= 128;
-  if (a->dtype == kFloat32)
-    return few ? (int)launch_pdl(tokens, rope_kv_write_int8_kernel<float, 4>, grid, dim3(128), shared, a->stream, p, chunk)
-               : (int)launch_pdl(tokens, rope_kv_write_int8_kernel<float, 8>, grid, dim3(256), shared, a->stream, p, chunk);
-  return few ? (int)launch_pdl(tokens, rope_kv_write_int8_kernel<bf16, 4>, grid, dim3(128), shared, a->stream, p, chunk)
-             : (int)launch_pdl(tokens, rope_kv_write_int8_kernel<bf16, 8>, grid, dim3(256), shared, a->stream, p, chunk);
+  if (a->dtype == kFloat32) return few ? launch_append<float, 4>(p, chunk, grid, shared, a->stream) : launch_append<float, 8>(p, chunk, grid, shared, a->stream);
+  return few ? launch_append<bf16, 4>(p, chunk, grid, shared, a->stream) : launch_append<bf16, 8>(p, chunk, grid, shared, a->stream);
 }
 
 struct ReadPagesInt8Args {
