@@ -219,7 +219,8 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     # The pages that the rest can see, in q's type, and a table of them, in one piece of memory.
     if every or (prompts and singles):
         rows, sequences, part = num_seqs, None, plan
-        longest = 0 if plan is None else max(plan.max_prefill_context_len, plan.max_decode_context_len)
+        known = [0] if plan is None else [plan.max_prefill_context_len] * (plan.num_prefill > 0) + [plan.max_decode_context_len] * (plan.num_decode > 0)
+        longest = max(known) if min(known) > 0 else 0
     elif prompts:
         rows, sequences, longest, part = prompts, plan.prefill_seqs, plan.max_prefill_context_len, plan
     else:
