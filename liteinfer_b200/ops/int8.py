@@ -158,7 +158,8 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     pages of a multiple of 16 tokens read the pages as they are; `decode_splits` blocks share a sequence's keys (rounded down to a
     power of two, 8 at most; None: chosen from the batch and the context).  Portions of prompts of these head and page sizes
     read whole numbers that are spread out to 16 bits first, exactly, and keep the scales apart.  For everything else the
-    pages that can be seen are read back into q's type once, and `paged_attention` runs over those.
+    pages that can be seen are read back into q's type once, and `paged_attention` runs over those.  Either is made room for by the
+    longest context of a launch; so many sequences go at a time as `WORK_BYTES` hold, one at least (`attention_int8_work`).
     """
     _rows2d(q, "q"); _rows2d(out, "out")
     _ints(block_table, query_start_loc, context_lens)
@@ -191,13 +192,16 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
         else:
             sequences, longest, most_queries = plan.prefill_seqs.data_ptr(), plan.max_prefill_context_len, plan.max_prefill_query_len
         blocks = min(-(-longest // page_size), most) if longest else most
-        size = prompts * blocks * kv_heads * page_size * (4 * head_dim + 1) + 128 + (q.shape[0] * heads * (4 * head_dim + 4) if dtype is torch.float32 else 0)
-        work = torch.empty((size,), dtype=torch.int8, device=q.device)
-        _check(_fn("li_attention_int8_prompt")(_ATTENTION_PROMPT(
-            code, q.data_ptr(), q.shape[0], q_row_stride, out.data_ptr(), out.stride(0), k, v, k_scale, v_scale, table, stride, starts, contexts,
-            sequences, prompts, most_queries, heads, kv_heads, head_dim, page_size, num_pages, scale, span, kept, softcap,
-            0 if sink is None else sink.data_ptr(), work.data_ptr(), blocks, _k.scratch_for(q.device).gemm_error.data_ptr(), stream)),
-            "paged_attention_int8")
+        each, rest = _spread_bytes(blocks * page_size, q.shape[0], heads, kv_heads, head_dim, dtype)
+        at_once = _at_once(prompts, each)
+        work = torch.empty((at_once * each + rest,), dtype=torch.int8, device=q.device)
+        for first in range(0, prompts, at_once):        # (in a list of sequences, or in the batch itself)
+            here = (table, starts, contexts, sequences + 4 * first) if sequences else (table + 4 * first * stride, starts + 4 * first, contexts + 4 * first, 0)
+            _check(_fn("li_attention_int8_prompt")(_ATTENTION_PROMPT(
+                code, q.data_ptr(), q.shape[0], q_row_stride, out.data_ptr(), out.stride(0), k, v, k_scale, v_scale, here[0], stride, here[1], here[2],
+                here[3], min(at_once, prompts - first), most_queries, heads, kv_heads, head_dim, page_size, num_pages, scale, span, kept, softcap,
+                0 if sink is None else sink.data_ptr(), work.data_ptr(), blocks, _k.scratch_for(q.device).gemm_error.data_ptr(), stream)),
+                "paged_attention_int8")
         prompts, beside = 0, most_queries > 0 and blocks > 0       # (the single tokens' kernel need not wait for this one, if there is one)
     # (Where `paged_attention` takes all sequences in one launch, it takes the single tokens next to portions too.)
     every = plan is None or not _k.mma_attention_supports(dtype, heads, kv_heads, head_dim)
@@ -217,29 +221,87 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
         return out
 
     # The pages that the rest can see, in q's type, and a table of them, in one piece of memory.
-    if every or (prompts and singles):
-        rows, sequences, part = num_seqs, None, plan
-        known = [0] if plan is None else [plan.max_prefill_context_len] * (plan.num_prefill > 0) + [plan.max_decode_context_len] * (plan.num_decode > 0)
-        longest = max(known) if min(known) > 0 else 0
-    elif prompts:
-        rows, sequences, longest, part = prompts, plan.prefill_seqs, plan.max_prefill_context_len, plan
-    else:
-        rows, sequences, longest, part = singles, plan.decode_seqs, plan.max_decode_context_len, plan
-    blocks = min(-(-longest // page_size), most) if longest else most
-    size = rows * blocks * kv_heads * page_size * head_dim * dtype.itemsize
-    work = torch.empty((2 * size + 4 * block_table.shape[0] * blocks,), dtype=torch.int8, device=q.device)
-    keys = work.data_ptr()
-    _check(_fn("li_read_pages_int8")(_READ_PAGES(
-        code, k, v, k_scale, v_scale, table, stride, contexts, keys, keys + size, rows, blocks, kv_heads, head_dim, page_size, num_pages,
-        0 if sequences is None else sequences.data_ptr(), starts, span, kept, keys + 2 * size, stream)), "read_pages_int8")
-    pools = work[:2 * size].view(dtype).view(2, rows * blocks, kv_heads, page_size, head_dim)
+    part = plan
     if part is not None and prompts != part.num_prefill:
         part = replace(part, num_prefill=0, prefill_seqs=None, max_prefill_query_len=0)
     if part is not None and singles != part.num_decode:
         part = replace(part, num_decode=0, decode_seqs=None, decode_tokens=None, decode_longest_first=None)
-    return _k.paged_attention(q, q_row_stride, out, pools[0], pools[1], work[2 * size:].view(torch.int32).view(-1, blocks), query_start_loc,
-                              context_lens, num_seqs, max_q_len, heads, kv_heads, head_dim, scale, window, plan=part,
-                              decode_splits=decode_splits, keep_first=keep_first, softcap=softcap, sink=sink, chunk=chunk)
+    options = dict(decode_splits=decode_splits, keep_first=keep_first, softcap=softcap, sink=sink, chunk=chunk)
+
+    def over_read_back(count, longest, part, sequences=None, first=0):
+        """Attention of `count` sequences of up to `longest` tokens (0: not known), the rows of the batch that `sequences` names or those from
+        `first` on."""
+        blocks = min(-(-longest // page_size), most) if longest else most
+        size = _read_back_bytes(count * blocks * page_size, kv_heads, head_dim, dtype)
+        rows = block_table.shape[0] - first
+        work = torch.empty((2 * size + 4 * rows * blocks,), dtype=torch.int8, device=q.device)
+        keys = work.data_ptr()
+        _check(_fn("li_read_pages_int8")(_READ_PAGES(
+            code, k, v, k_scale, v_scale, table + 4 * first * stride, stride, contexts + 4 * first, keys, keys + size, count, blocks, kv_heads, head_dim,
+            page_size, num_pages, 0 if sequences is None else sequences.data_ptr(), starts + 4 * first, span, kept, keys + 2 * size, stream)),
+            "read_pages_int8")
+        pools = work[:2 * size].view(dtype).view(2, count * blocks, kv_heads, page_size, head_dim)
+        _k.paged_attention(q, q_row_stride, out, pools[0], pools[1], work[2 * size:].view(torch.int32).view(-1, blocks), query_start_loc[first:],
+                           context_lens[first:], count if sequences is None else num_seqs, max_q_len, heads, kv_heads, head_dim, scale, window, plan=part,
+                           **options)
+
+    def room_for(count, longest):
+        return _at_once(count, 2 * _read_back_bytes(min(longest, most * page_size) if longest else most * page_size, kv_heads, head_dim, dtype))
+
+    known = [0] if plan is None else [plan.max_prefill_context_len] * (plan.num_prefill > 0) + [plan.max_decode_context_len] * (plan.num_decode > 0)
+    whole = max(known) if min(known) > 0 else 0
+    if every or (prompts and singles and room_for(num_seqs, whole) >= num_seqs):
+        # (A plan that deals the sequences to launches of their own goes with all of them.)
+        at_once = room_for(num_seqs, whole)
+        for first in range(0, num_seqs, at_once):
+            over_read_back(min(at_once, num_seqs - first), whole, part, first=first)
+        return out
+    no_portions = dict(num_prefill=0, prefill_seqs=None, max_prefill_query_len=0)
+    no_singles = dict(num_decode=0, decode_seqs=None, decode_tokens=None, decode_longest_first=None)
+    if prompts:
+        at_once = room_for(prompts, plan.max_prefill_context_len)
+        for first in range(0, prompts, at_once):
+            rows, count = plan.prefill_seqs[first:first + at_once], min(at_once, prompts - first)
+            over_read_back(count, plan.max_prefill_context_len, replace(plan, num_prefill=count, prefill_seqs=rows, **no_singles), rows)
+    if singles:
+        at_once = room_for(singles, plan.max_decode_context_len)
+        for first in range(0, singles, at_once):
+            some = slice(first, first + at_once)
+            mine = replace(plan, **no_portions)
+            if at_once < singles:
+                mine = replace(mine, num_decode=min(at_once, singles - first), decode_seqs=plan.decode_seqs[some], decode_tokens=plan.decode_tokens[some],
+                               decode_longest_first=None)
+            over_read_back(mine.num_decode, plan.max_decode_context_len, mine, mine.decode_seqs)
+    return out
+
+
+# The most memory that a call of `paged_attention_int8` takes to spread pages out or to read them back, but for a single sequence of a launch,
+# which it takes whole.
+WORK_BYTES = 1 << 30
+
+
+def _spread_bytes(context: int, tokens: int, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
+    """What a portion of a context takes spread out to 16 bits, and what its launch takes besides (li_attention_int8_prompt)."""
+    return context * kv_heads * (4 * head_dim + 1), 128 + (tokens * heads * (4 * head_dim + 4) if dtype is torch.float32 else 0)
+
+
+def _read_back_bytes(tokens: int, kv_heads: int, head_dim: int, dtype: torch.dtype) -> int:
+    """What keys (or values) of this many tokens take in q's type."""
+    return tokens * kv_heads * head_dim * dtype.itemsize
+
+
+def _at_once(count: int, each: int) -> int:
+    """How many of `count` sequences go at a time."""
+    return max(1, min(count, WORK_BYTES // max(1, each)))
+
+
+def attention_int8_work(sequences: int, context: int, tokens: int, heads: int, kv_heads: int, head_dim: int, page_size: int, dtype: torch.dtype) -> int:
+    """The most bytes that a call of `paged_attention_int8` takes beside its arguments, over `sequences` of up to `context` tokens that bring
+    `tokens` in all."""
+    context = -(-context // page_size) * page_size
+    spread, rest = _spread_bytes(context, tokens, heads, kv_heads, head_dim, dtype)
+    read_back = 2 * _read_back_bytes(context, kv_heads, head_dim, dtype)
+    return max(_at_once(sequences, spread) * spread + rest, _at_once(sequences, read_back) * read_back + 4 * sequences * context // page_size)
 
 
 _supported: dict[tuple[str, int, int, int, int], bool] = {}
