@@ -257,6 +257,12 @@ class Attention:
             bounds = tuple(sorted({*bounds, 1024, 4096, 16384, 65536}))
         return bounds
 
+    def work_bytes(self, sequences: int, context: int, tokens: int, page_size: int, dtype: torch.dtype) -> int:
+        """Memory that a step takes here beside its activations, with so many sequences of so long contexts that bring so many tokens."""
+        if not self.int8_cache:
+            return 0
+        return ops.attention_int8_work(sequences, context, tokens, self.heads, self.kv_heads, self.head_dim, page_size, dtype)
+
     def forward(self, x, ctx: StepContext, cache: LayerCache, residual: torch.Tensor | None = None):
         if self.qkv_int8 is not None:
             x = x.materialise() if isinstance(x, ops.PendingNorm) else x

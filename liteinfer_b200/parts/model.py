@@ -166,6 +166,12 @@ class Model:
                         seen[one.data_ptr()] = one.numel() * one.element_size()
         return sum(seen.values())
 
+    def work_bytes(self, sequences: int, context: int, tokens: int, page_size: int) -> int:
+        """The most memory that a part takes in a step beside activations, with up to so many sequences of so long contexts that bring so many
+        tokens."""
+        return max((part.work_bytes(sequences, context, tokens, page_size, self.dtype) for _, part, _ in self._named_parts()
+                    if hasattr(part, "work_bytes")), default=0)
+
     # --------------------------------------------------------------- cache
     def cache_needs(self) -> list[tuple]:
         """What each layer (by index) must keep between steps."""
