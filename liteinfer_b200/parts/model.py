@@ -142,6 +142,7 @@ class Model:
                 part.hold_in_int8(weights, cache)
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)      # the weights are at rest from here on
+            torch.cuda.empty_cache()                 # what they took before is the device's again, and the pages'
 
     @property
     def graph_safe(self) -> bool:
