@@ -350,6 +350,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   auto empty = [&](int s) { return bars + 8u * (kSlots + s); };
   const unsigned q_full = bars + 8u * (2 * kSlots);
   auto tile_bar = [&](int x, int which) { return q_full + 8u * (1 + x * 3 + which); };
+  const unsigned drained = tile_bar(X, 0);
   __shared__ unsigned tmem_slot;
   __shared__ float between[X][kRows];       // a row's two threads
   unsigned char* generic_base = smem_raw + (base - smem_addr(smem_raw));
@@ -387,6 +388,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       mbar_init(empty(s), 1);
     }
     mbar_init(q_full, 1);
+    mbar_init(drained, 1);
     for (int t = 0; t < X; ++t) {
       mbar_init(tile_bar(t, 0), 1);
       mbar_init(tile_bar(t, 1), 8);
@@ -435,9 +437,11 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
 
   if (warp == 0) {
     // ------------------------------------------------------------------ loader
-    for (int i = ahead; i < 2 * ntiles; ++i)
-      if (!load_slot(i, false)) break;
-    if (kSplit && ntiles == 0) warp_wait(q_full, 0, p.error_flag, 54);       // (nobody leaves before what was asked for has come)
+    int asked = ahead;
+    while (asked < 2 * ntiles && load_slot(asked, false)) ++asked;
+    // Nobody leaves before what was asked for has come, also where there was nothing to do with it or a wait gave up.
+    warp_wait(q_full, 0, p.error_flag, 54);
+    for (int i = max(0, asked - kSlots); i < asked; ++i) warp_wait(full(i % kSlots), (unsigned)(i / kSlots) & 1, nullptr, 0);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ issuer
     {
@@ -493,6 +497,10 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
           ok = issue_pv(t, tile);
           if (ok && t + 1 < ntiles) issue_qk(t + 1, tile);
         }
+      }
+      if (!ok && ntiles > 0) {        // products that are under way still are done before tensor memory goes back
+        if (elected()) umma_commit(drained);
+        warp_wait(drained, 0, nullptr, 0);
       }
     }
   } else if (warp >= 4) {
@@ -782,7 +790,7 @@ static bool tile_map(CUtensorMap* map, const void* ptr, long rows, int head_dim,
 template <int D, int X, bool kCapped, bool kTwo, bool kSplit>
 static int launch_prompt_as(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PromptParams& p, dim3 grid, cudaStream_t stream) {
   constexpr int kTiles = kTwo ? 2 : X, kSlots = PromptSlots<D, kTiles>::value, kScaleSlots = PromptScales<D>::value;
-  constexpr size_t smem = (size_t)kTiles * kRows * D * 2 + kSlots * (size_t)kKeys * D * 2 + kScaleSlots * kRuns * 16 + 8 * (2 * kSlots + 1 + 3 * X) + 1024;
+  constexpr size_t smem = (size_t)kTiles * kRows * D * 2 + kSlots * (size_t)kKeys * D * 2 + kScaleSlots * kRuns * 16 + 8 * (2 * kSlots + 2 + 3 * X) + 1024;
   static_assert(smem + X * 4 * kRows + 16 <= 232448, "more shared memory than a block may have");
   static_assert(!kSplit || (D + 2) * kRows * 4 <= kSlots * kKeys * D * 2, "sums where the ring was");
   auto kernel = attention_int8_prompt_kernel<D, X, kCapped, kTwo, kSplit>;

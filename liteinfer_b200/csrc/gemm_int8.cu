@@ -549,15 +549,18 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
       grid_launch_dependents();
       grid_dependency_wait();
       for (int i = 0; i < early; ++i) tma_load_2d(base + i * stage_bytes + kBytesW, &map_x, full_bar(i), (kb_lo + i) * kTileK, m0);
-      int stage = 0;
+      int stage = 0, asked = early;
       unsigned phase = 1;
       for (int kb = kb_lo + early; kb < kb_hi; ++kb) {
         if (!mbar_wait(empty_bar(stage), phase ^ 1, p.error_flag, 42)) { failed = 1; break; }
         mbar_expect_tx(full_bar(stage), stage_bytes);
         tma_load_2d(base + stage * stage_bytes, &map_w, full_bar(stage), kb * kTileK, n0);
         tma_load_2d(base + stage * stage_bytes + kBytesW, &map_x, full_bar(stage), kb * kTileK, m0);
+        ++asked;
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
+      // What was asked for lands before the block ends, also where a wait gave up (the issuer's, say).
+      for (int i = max(0, asked - p.stages); i < asked; ++i) mbar_wait(full_bar(i % p.stages), (unsigned)(i / p.stages) & 1, nullptr, 0);
     }
   } else if (warp == 1) {
     const unsigned idesc = i8_desc(kTileRows, p.cols);
@@ -683,7 +686,7 @@ constexpr int kPairWarps = 12;             // that empty the accumulators
 constexpr int kPairThreads = 64 + 32 * kPairWarps;
 constexpr int kTurnRow = 40;               // bfloat16 of a row being turned: 32 and the padding that keeps 16-byte alignment
 constexpr unsigned kPairStage = kBytesW + 128 * kTileK;
-constexpr size_t kPairSmem = 1024 + kPairStages * kPairStage + kPairWarps * 32 * kTurnRow * 2 + 8 * (2 * kPairStages + 4);
+constexpr size_t kPairSmem = 1024 + kPairStages * kPairStage + kPairWarps * 32 * kTurnRow * 2 + 8 * (2 * kPairStages + 5);
 
 // Tiles are walked in bands of eight tiles of w, x's tiles side by side inside a band, so that the pairs running at the same time
 // share a few tiles of either (which then come from L2).
@@ -706,6 +709,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   auto empty_bar = [&](int s) { return bars + 8u * (kPairStages + s); };      // signalled in both CTAs
   auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kPairStages + b); };         // signalled in both CTAs
   auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kPairStages + 2 + b); };    // the leader's: both CTAs' warps arrive
+  const unsigned drained_bar = bars + 8u * (2 * kPairStages + 4);                       // signalled in both CTAs
   __shared__ unsigned tmem_slot;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -726,6 +730,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       mbar_init(acc_full_bar(b), 1);
       mbar_init(acc_empty_bar(b), 2 * kPairWarps);
     }
+    mbar_init(drained_bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {   // the same warp in both CTAs: the allocation is made for the pair
@@ -741,7 +746,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 
   if (warp == 0) {
     if (lane == 0) {
-      int stage = 0;
+      int stage = 0, asked = 0;
       unsigned phase = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < num_tiles; tile += pairs) {
@@ -753,9 +758,13 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
           const unsigned a = base + stage * kPairStage;
           tma_load_2d_pair(a, &map_w, full_bar(stage), kb * kTileK, tn * 2 * kTileRows + (int)rank * kTileRows);
           tma_load_2d_pair(a + kBytesW, &map_x, full_bar(stage), kb * kTileK, tm * p.cols + (int)rank * (p.cols / 2));
+          ++asked;
           if (++stage == kPairStages) { stage = 0; phase ^= 1; }
         }
       }
+      // What either CTA asked for lands before the pair ends, also where a wait gave up.
+      if (rank == 0)
+        for (int i = max(0, asked - kPairStages); i < asked; ++i) mbar_wait(full_bar(i % kPairStages), (unsigned)(i / kPairStages) & 1, nullptr, 0);
     }
   } else if (warp == 1) {
     // The whole warp goes along and one of its lanes issues: a lane that is alone in a branch takes some 100 cycles a product for it, as much
@@ -785,6 +794,10 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
           __syncwarp();
           if (++stage == kPairStages) { stage = 0; phase ^= 1; }
         }
+      }
+      if (!ok) {        // products that are under way still are done before tensor memory goes back
+        if (elected()) umma_commit_pair(drained_bar);
+        warp_wait(drained_bar, 0, nullptr, 0);
       }
     }
   } else {
