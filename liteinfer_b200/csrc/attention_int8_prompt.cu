@@ -43,7 +43,8 @@ struct ExpandParams {
   const int* context_lens;
   const int* row_index;     // optional: batch row of each portion (negative: none)
   int window, keep_first;
-  float score;              // scale * log2(e), or with capped scores scale / cap
+  float score;              // |scale| * log2(e), or with capped scores |scale| / cap
+  unsigned flip;            // what turns two keys' signs where the scale is negative (the softmax wants factors that are not), else 0
   uint4* out[2];            // [rows][kv_heads][blocks * page_size][head_dim] of 16 bits
   float4* runs;             // [rows][kv_heads][blocks * page_size / 16]: f, lv, 2^-lv, 2^lv of 16 tokens
   int blocks, kv_heads, head_dim, page_size, num_pages;
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(256) expand_pages_int8_kernel(const ExpandPara
   }
   const int vectors = p.page_size * p.head_dim / 16;      // of a head
   const bool halves = which || p.half_keys;
+  const unsigned flip = which ? 0u : p.flip;
   const uint4* in = reinterpret_cast<const uint4*>(p.pool[which]) + from * vectors;
 #pragma unroll 4
   for (int v = part * (int)blockDim.x + threadIdx.x; v < p.kv_heads * vectors; v += parts * (int)blockDim.x) {
@@ -100,8 +102,8 @@ __global__ void __launch_bounds__(256) expand_pages_int8_kernel(const ExpandPara
     unsigned r[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      r[2 * e] = halves ? as_halves(w[e]) : as_bfloats(w[e]);
-      r[2 * e + 1] = halves ? as_halves(w[e] >> 16) : as_bfloats(w[e] >> 16);
+      r[2 * e] = (halves ? as_halves(w[e]) : as_bfloats(w[e])) ^ flip;
+      r[2 * e + 1] = (halves ? as_halves(w[e] >> 16) : as_bfloats(w[e] >> 16)) ^ flip;
     }
     uint4* out = p.out[which] + ((((size_t)i * p.kv_heads + h) * p.blocks + b) * vectors + (v - h * vectors)) * 2;
     out[0] = make_uint4(r[0], r[1], r[2], r[3]);
@@ -877,7 +879,7 @@ LI_EXPORT int li_attention_int8_prompt(const AttentionInt8PromptArgs* a) {
   const int keep_first = a->window > 0 ? (int)a->keep_first : 0;
   ExpandParams e{{(const signed char*)a->k_pool, (const signed char*)a->v_pool}, {a->k_scale, a->v_scale}, a->block_table,
                  (int)a->table_stride, a->query_start_loc, a->context_lens, a->seq_index, (int)a->window, keep_first,
-                 capped ? (float)(a->scale / a->softcap) : (float)a->scale * kLog2eF, {(uint4*)work, (uint4*)(work + bytes)},
+                 fabsf(capped ? (float)(a->scale / a->softcap) : (float)a->scale * kLog2eF), a->scale < 0 ? 0x80008000u : 0u, {(uint4*)work, (uint4*)(work + bytes)},
                  (float4*)(work + 2 * bytes), blocks, kv_heads, D, page_size, (int)a->num_pages, two_pieces};
   long long parts = 1;      // a page is a block's, and of several while they are not many a multiprocessor (1,024 queries behind 3,000, 32 heads on 8
                             // of 128: the call takes 84 us with a block a page, 80 with four)
