@@ -88,7 +88,9 @@ __global__ void __launch_bounds__(256) expand_pages_int8_kernel(const ExpandPara
     const float log2_v = log2f(v), lv = v == 0.f ? -60.f : log2_v < -90.f ? -90.f : log2_v;
     const int runs = p.page_size / 16;
     float4* out = p.runs + (((size_t)i * p.kv_heads + threadIdx.x) * p.blocks + b) * runs;
-    for (int g = 0; g < runs; ++g) out[g] = make_float4(k * p.score, lv, exp2f(-lv), lv == log2_v ? v : exp2f(lv));
+    // (tokens of no page weigh nothing)
+    for (int g = 0; g < runs; ++g)
+      out[g] = page < 0 ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(k * p.score, lv, exp2f(-lv), lv == log2_v ? v : exp2f(lv));
   }
   const int vectors = p.page_size * p.head_dim / 16;      // of a head
   const bool halves = which || p.half_keys;
@@ -590,7 +592,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
           if constexpr (kTwo) c.x *= q_factor;
           const Terms e = enter_run<kCapped>(v, c, kCapped || !all_seen, seen[g / 2] >> (g % 2 * 16), p.cap);
           // (Of 32 bits, 2^d comes as a factor behind the exponential: the sum of d and r would be rounded.)
-          const float d = kTwo ? 0.f : e.d;
+          const float d = kTwo && e.d != -INFINITY ? 0.f : e.d;
           const float2 factor = both(e.f), shift = both(r == -INFINITY ? d : d - r);
           float2 part = both(0.f);
 #pragma unroll
