@@ -168,6 +168,9 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
     code = _code(q)
     _refuse(dtype is not out.dtype or out.shape[1] != heads * head_dim, "out is [tokens, heads * head_dim] of q's type")
     _refuse(heads % kv_heads != 0, "the query heads are a multiple of the KV heads")
+    _refuse(q.shape[1] < heads * head_dim, f"a row of q has {q.shape[1]} numbers, fewer than its heads need")
+    _refuse(num_seqs > block_table.shape[0] or num_seqs > context_lens.numel() or num_seqs >= query_start_loc.numel(),
+            "every sequence has a row of the block table, a length and a start, the last one an end")
     if sink is not None:
         _on_gpu(sink)
         _refuse(sink.dtype is not torch.float32 or sink.numel() != heads, "a sink is float32, one number a head")
