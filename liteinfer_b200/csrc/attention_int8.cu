@@ -1,5 +1,5 @@
-// Paged attention of single decoded tokens over keys and values held in 8 bits (int8_cache.cu); prompts and portions read their pages
-// back first and take the kernels of 16 and 32 bits (ops/int8.py).
+// Paged attention of single decoded tokens over keys and values held in 8 bits (int8_cache.cu); portions of prompts are
+// attention_int8_prompt.cu's, and sizes that neither takes read their pages back and go to the kernels of 16 and 32 bits (ops/int8.py).
 //
 //   out = sum_j w_j s_v(page of j) v_j / sum_j w_j,   w_j = exp(scale * s_k(page of j) * (q . k_j) - max),
 //

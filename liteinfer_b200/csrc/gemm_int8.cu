@@ -7,7 +7,7 @@
 // products are rounded in the order given and the result once more to the engine's type.
 //
 // Three kernels, by the number of rows of x (see li_linear_int8 for the rule).  Each of them starts while the quantisation ahead of it
-// still runs (programmatic dependent launch) and asks for its first weights before it waits for it.
+// still runs (programmatic dependent launch); the first two ask for their first weights before they wait for it.
 //   stream   few rows: the time is that of reading w once; per-warp rings of TMA copies, mma.sync m16n8k32
 //   cluster  some rows, or few tiles: one 128 x 256 tile a cluster of up to four CTAs that share its k (tcgen05 kind::i8), their
 //            sums added up through distributed shared memory

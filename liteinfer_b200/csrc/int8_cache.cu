@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
   const int half = p.inv_freq != nullptr ? p.rotary_dim / 2 : 0, D = p.head_dim, units = D / 16;
   const int t0 = blockIdx.x * chunk, mine = min(chunk, p.tokens - t0);
   grid_dependency_wait();
-  // Only now may the kernel behind start: the attention reads pages of which none is written any more but those of this launch.
+  // Only now may the kernel behind start: what came before this launch is done, and the attention of single tokens may read, while this one
+  // still writes, the pages that it does not touch.
   grid_launch_dependents();
   const T* const rows = (const T*)p.qkv + (size_t)t0 * p.row_stride;
   int from = 0, reach = mine;             // tokens whose angles are needed

@@ -137,8 +137,7 @@ class EngineCore:
         widest = min(cfg.token_budget, cfg.max_num_seqs * cfg.max_model_len)
         activations = widest * model.spec.hidden_size * element * 32 + cfg.max_num_seqs * model.spec.vocab_size * 8
         states = CacheManager.state_bytes_for(model.cache_needs(), model.schedule, cfg.max_num_seqs, cfg.dtype)
-        # A part's work space: once for steps run kernel by kernel; graphs share a pool, in which smaller shapes' may lie beside the largest's,
-        # each at most half of the next.
+        # A part's work space: once for steps run kernel by kernel, twice for graphs, in whose pool smaller shapes' may lie beside the largest's.
         work = 3 * model.work_bytes(cfg.max_num_seqs, cfg.max_model_len, widest, cfg.block_size)
         budget = free - int(total * (1.0 - cfg.gpu_memory_utilization)) - activations - states - work
         affordable = max(0, budget // per_page)
