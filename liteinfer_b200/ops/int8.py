@@ -205,6 +205,7 @@ def paged_attention_int8(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, 
                 here[3], min(at_once, prompts - first), most_queries, heads, kv_heads, head_dim, page_size, num_pages, scale, span, kept, softcap,
                 0 if sink is None else sink.data_ptr(), work.data_ptr(), blocks, _k.scratch_for(q.device).gemm_error.data_ptr(), stream)),
                 "paged_attention_int8")
+        del work                        # (what follows on the stream may have its place)
         prompts, beside = 0, most_queries > 0 and blocks > 0       # (the single tokens' kernel need not wait for this one, if there is one)
     # (Where `paged_attention` takes all sequences in one launch, it takes the single tokens next to portions too.)
     every = plan is None or not _k.mma_attention_supports(dtype, heads, kv_heads, head_dim)

@@ -50,3 +50,23 @@ def test_as_many_sequences_at_a_time_as_there_is_room_for(monkeypatch, layout, r
     _check_attention(MIXED + SINGLES, *layout, dtype)
     _check_attention(MIXED, *layout, dtype, planned=False)
     _check_attention(MIXED + SINGLES, *layout, dtype, window=40, keep_first=7)
+
+
+def test_portions_and_single_tokens_take_their_work_spaces_in_turn(monkeypatch):
+    """Behind kept first keys a step's portions are spread out and its single tokens' pages read back: one work space at a time."""
+    monkeypatch.setattr(int8, "WORK_BYTES", 200_000_000)
+    heads, kv_heads, dim, page, dtype = 8, 8, 128, 16, torch.bfloat16
+    sequences = [(20000, 5)] * 6 + [(20000, 1)] * 6
+    positions, seq, table, starts, context, total = _batch(sequences, page, 1)
+    pages = _pages(total, kv_heads, page, dim, 1)
+    q = torch.randn((positions.numel(), heads * dim), generator=_generator(2), device=DEVICE).to(dtype)
+    out = torch.empty_like(q)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEVICE)
+    plan = AttentionPlan(6, ints(list(range(6, 12))), ints(list(range(30, 36))), None, 6, ints(list(range(6))), 5, 20001, 20005)
+    kernels.scratch_for(DEVICE)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.paged_attention_int8(q, q.stride(0), out, pages, table, starts, context, 12, 5, heads, kv_heads, dim, dim ** -0.5, window=15000, keep_first=4, plan=plan)
+    most = ops.attention_int8_work(12, 20005, q.shape[0], heads, kv_heads, dim, page, dtype)
+    assert torch.cuda.max_memory_allocated() - before <= most + (1 << 23), (torch.cuda.max_memory_allocated() - before, most)
